@@ -48,13 +48,14 @@ __device__ __forceinline__ f2 exp2_2(f2 a)
 // 2^x of a pair to half a step of fp32, without the exponential unit: x = n + f, n the nearest integer (added and taken away with
 // 1.5 * 2^23, which leaves n in the low bits), f in [-1/2, 1/2]; 2^f by its minimax polynomial of degree 6 with constant term 1
 // (relative error 2^-28.9, and exact at 0, where the decays of slow states lie), times the float whose exponent field is n + 127. (An
-// integer addition of n to the polynomial's exponent would save that multiplication, but turns NaN into a number.) Below 2^-126 the
-// result stays 2^-126, from x = 127.5 on it is infinite, NaN stays NaN.
+// integer addition of n to the polynomial's exponent would save that multiplication, but turns NaN into a number.) Below x = -126.5 that
+// field is 0 and the result zero: a decay that forgets the state leaves nothing of it for A, which may be as large as floats go, to
+// magnify in the gradients. From x = 127.5 on the result is infinite, NaN stays NaN.
 __device__ __forceinline__ f2 exp2_poly_2(f2 x)
 {
 	float2 v = unpack2(x);
-	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
-	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
+	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.f));
+	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.f));
 	asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(128.f));
 	asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(128.f));
 	const f2 c = pack2(v.x, v.y);
