@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 					const float2 s = unpack2(t_r[e * RS]);
 					const float dl = unpack2(t_p[e * PS].x).x;
 					ox[e] = t_skip[e] * ds[e] + dl * s.x;
-					od[e] = s.y * (1.f / kLog2e) + xv[e] * s.x;
+					// A step that softplus left at zero has no gradient. The sum over A does not enter then: where A is the type's lowest value
+					// it overflows, and softplus' = 0 would turn that into NaN.
+					od[e] = (in.softplus && dl == 0.f ? 0.f : s.y * (1.f / kLog2e)) + xv[e] * s.x;
 					if (in.softplus) od[e] *= dv[e];
 					s_acc[e * 32 + lane] += ds[e] * xv[e];
 					s_acc[(EPT + e) * 32 + lane] += od[e];

@@ -66,3 +66,41 @@ def test_single_tokens_forget(ops, dtype):
     assert not state[:, 3].any()
     cut = {k: (v[:, 4:5] if k in ("x", "dt", "B", "C", "z") else v) for k, v in p.items()}
     assert not ops.tensor_selective_scan(**cut)[1][:, 3].any()
+
+
+@pytest.mark.parametrize("shape", [(2, 50, 24, 1, 16), (1, 700, 8, 1, 16), (2, 37, 6, 1, 5)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("mask", ["inf", "max"])
+def test_masked_tokens_of_channels_that_forget(ops, shape, dtype, mask):
+    """A step of zero passes state and adjoint on whatever A is, and its own gradient is zero: A g h, which overflows where A is the
+    type's lowest value, comes with softplus' = 0."""
+    b, l, d, g, n = shape
+    p, gen = inputs(17 + l, b, l, d, g, n, dtype)
+    p["A"][3], p["A"][5, 2] = LOWEST, LOWEST
+    masked = torch.rand(b, l, device="cuda", generator=gen) < 0.4
+    masked[:, -1] = False
+    p["dt"][masked] = -float("inf") if mask == "inf" else torch.finfo(dtype).min
+    p["initial_states"] *= 100
+    dy, dfin = rn(gen, b, l, d, dtype=dtype) * 8, rn(gen, b, d, n) * 100
+    y, fin, ck = ops.tensor_selective_scan(**p, want_checkpoints=True)
+    grads = ops.tensor_selective_scan_backward(dy, checkpoints=ck, dfinal_states=dfin, **p)
+    for name, _ in GRADS:
+        assert torch.isfinite(getattr(grads, name)).all(), name
+    assert not grads.ddt[masked].any() and not grads.dB[masked].any()
+    # where dy is zero too, a masked token is as good as not there
+    dy[masked] = 0
+    grads = ops.tensor_selective_scan_backward(dy, checkpoints=ck, dfinal_states=dfin, **p)
+    for i in range(b):
+        kept = ~masked[i]
+        row = lambda k, v: v[i:i + 1, kept].contiguous() if k in ("x", "dt", "B", "C", "z") else (v[i:i + 1] if k == "initial_states" else v)
+        one = {k: row(k, v) for k, v in p.items()}
+        leaves = {k: v.requires_grad_() for k, v in reference_args(one).items()}
+        wy, wfin = ref.scan(**leaves)
+        dyi, dfi = dy[i:i + 1, kept].double(), dfin[i:i + 1].double()
+        ((wy * dyi).sum() + (wfin * dfi).sum()).backward()
+        bounds = ref.scan_bounds(**reference_args(one), dy=dyi, dfin=dfi)
+        for j, (name, leaf) in enumerate(GRADS):
+            if leaf in ("x", "dt", "B", "C", "z"):
+                ref.assert_within(getattr(grads, name)[i:i + 1, kept], leaves[leaf].grad, bounds[2 + j], name)
+            elif leaf == "init":
+                ref.assert_within(grads.dinitial_states[i:i + 1], leaves[leaf].grad, bounds[2 + j], name)
