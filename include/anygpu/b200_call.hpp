@@ -44,3 +44,17 @@ inline void* b200_workspace(const size_t bytes)
 	}
 	return ws[dev]->buffer;
 }
+
+// Whether the dimensions of t behind the first `lead` are dense, as a template relies on that hands the kernels a row stride only.
+// Dimensions of one entry have no stride of their own.
+template <typename dtype>
+inline bool b200_dense(const Tensor<dtype, CUDA>& t, const int64 lead)
+{
+	int64 expect = 1;
+	for (int64 i = t.dim - 1; i >= lead; --i)
+	{
+		if (t.shape[i] != 1 && t.stride[i] != expect) return false;
+		expect *= t.shape[i];
+	}
+	return true;
+}

@@ -1,7 +1,7 @@
 // Selective scan with a decay per channel and state (the form of state-space layers before the per-head scan of mamba_chunk_scan.hpp):
 // x, dt, z (b,l,dim), A (dim,n), B/C (b,l,g,n), D and dt_bias (dim), initial_states (b,dim,n); softplus of the step sizes is on. A, D,
-// dt_bias and all states are float32. Activations may be last-axis slice views of wider tensors (evenly spaced rows). No counterpart in
-// anyGPU.
+// dt_bias and all states are float32. Activations may be last-axis slice views of wider tensors (evenly spaced rows); of B and C that
+// holds for whole rows of g * n elements, not for some of the states of every group. No counterpart in anyGPU.
 #pragma once
 
 #include "../b200_call.hpp"
@@ -24,8 +24,8 @@ struct SelectiveScanArgs
 		ACASSERT(x.dim == 3 && dt.dim == 3 && B.dim == 4 && C.dim == 4 && A.dim == 2, "x, dt (b,l,dim), A (dim,n), B/C (b,l,g,n)");
 		const int64 b = x.shape[0], l = x.shape[1], d = x.shape[2], g = B.shape[2], n = B.shape[3];
 		ACASSERT(A.shape[0] == d && A.shape[1] == n && C.shape[2] == g && C.shape[3] == n, "A, B and C do not match");
-		auto rows = [&](const auto& t) { return t.shape[0] == b && t.shape[1] == l && t.stride[0] == l * t.stride[1]; };
-		ACASSERT(rows(x) && rows(dt) && rows(B) && rows(C) && (!z || rows(*z)), "batch or length do not match, or rows are not evenly spaced");
+		auto rows = [&](const auto& t) { return t.shape[0] == b && t.shape[1] == l && t.stride[0] == l * t.stride[1] && b200_dense(t, 2); };
+		ACASSERT(rows(x) && rows(dt) && rows(B) && rows(C) && (!z || rows(*z)), "batch or length do not match, or rows are not evenly spaced and dense");
 		ACASSERT(dt.shape[2] == d && (!z || (z->dim == 3 && z->shape[2] == d)), "dt or z does not match x");
 		ACASSERT((!D || D->numel() == d) && (!dt_bias || dt_bias->numel() == d), "D or dt_bias does not match x");
 		ACASSERT(!initial_states || initial_states->numel() == b * d * n, "initial_states does not match");
@@ -75,6 +75,7 @@ inline Tensor<dtype, CUDA> tensor_selective_scan_update(Tensor<float32, CUDA>& s
 	ACASSERT(dt.shape[0] == b && dt.shape[1] == d && B.shape[0] == b && C.shape[0] == b, "dt, B or C does not match x");
 	ACASSERT((!z || (z->dim == 2 && z->shape[0] == b && z->shape[1] == d)) && (!D || D->numel() == d) && (!dt_bias || dt_bias->numel() == d),
 		"z, D or dt_bias does not match x");
+	ACASSERT(b200_dense(x, 1) && b200_dense(dt, 1) && b200_dense(B, 1) && b200_dense(C, 1) && (!z || b200_dense(*z, 1)), "rows are not dense");
 	Tensor<dtype, CUDA> y(x.dim, x.shape);
 	b200_check(b200_selective_scan_update(b200_dtype_of<dtype>(), state.buffer(), x.buffer(), x.stride[0], dt.buffer(), dt.stride[0], A.buffer(), 0,
 		B.buffer(), B.stride[0], C.buffer(), C.stride[0], D ? D->buffer() : nullptr, dt_bias ? dt_bias->buffer() : nullptr, z ? z->buffer() : nullptr,
@@ -95,8 +96,8 @@ inline SelectiveScanGradients<dtype> tensor_selective_scan_backward(const Tensor
 	const Tensor<float32, CUDA>& checkpoints, const Tensor<float32, CUDA>* dfinal_states = nullptr)
 {
 	const b200_selective_scan_inputs in = args.c_struct();
-	ACASSERT(dy.dim == 3 && dy.shape[0] == in.batch && dy.shape[1] == in.seqlen && dy.shape[2] == in.dim && dy.stride[0] == in.seqlen * dy.stride[1],
-		"dy does not match x");
+	ACASSERT(dy.dim == 3 && dy.shape[0] == in.batch && dy.shape[1] == in.seqlen && dy.shape[2] == in.dim && dy.stride[0] == in.seqlen * dy.stride[1] &&
+		b200_dense(dy, 2), "dy does not match x");
 	ACASSERT(static_cast<size_t>(checkpoints.numel()) * sizeof(float) == b200_selective_scan_checkpoint_bytes(in.batch, in.seqlen, in.dim, in.d_state),
 		"checkpoints are not of this call");
 	ACASSERT(!dfinal_states || dfinal_states->numel() == in.batch * in.dim * in.d_state, "dfinal_states does not match");
