@@ -58,3 +58,12 @@ inline bool b200_dense(const Tensor<dtype, CUDA>& t, const int64 lead)
 	}
 	return true;
 }
+
+// Whether the rows of t (over its first `lead` dimensions) are evenly spaced, stride[lead - 1] apart, and dense.
+template <typename dtype>
+inline bool b200_even_rows(const Tensor<dtype, CUDA>& t, const int64 lead)
+{
+	for (int64 i = lead - 2; i >= 0; --i)
+		if (t.shape[i] != 1 && t.stride[i] != t.shape[i + 1] * t.stride[i + 1]) return false;
+	return b200_dense(t, lead);
+}

@@ -24,7 +24,7 @@ inline Tensor<dtype, CUDA> tensor_rms_norm(const Tensor<dtype, CUDA>& xt, const 
 }
 
 // tensor_layer_norm for CUDA tensors, float16 and float32 (anyGPU srcs/ops/norm_ops.hpp; its CUDA kernel is float32 only), over the last
-// axis: (x - mean) / sqrt(var + eps) * w + b. xt may be a slice view of a wider tensor. tensor_layer_norm_with_stats also returns the
+// axis: (x - mean) / sqrt(var + eps) * w + b. xt may be a last-axis slice view of a wider tensor. tensor_layer_norm_with_stats also returns the
 // fp32 mean and 1 / sqrt(var + eps) of every row, which the backward call needs.
 template <typename dtype>
 struct LayerNormResult
@@ -42,6 +42,7 @@ inline LayerNormResult<dtype> tensor_layer_norm_with_stats(const Tensor<dtype, C
 	ACASSERT((dim + axis) % dim == dim - 1, "the norm region is the last axis");
 	const int64 d = xt.shape[dim - 1];
 	ACASSERT(wt.shape[0] == d && bt.shape[0] == d, "wt or bt shape is incorrect");
+	ACASSERT(b200_even_rows(xt, dim - 1), "the rows of xt need to be evenly spaced and dense");
 	const int64 rows = xt.numel() / d, xs = dim >= 2 ? xt.stride[dim - 2] : d;
 	LayerNormResult<dtype> r{ Tensor<dtype, CUDA>(dim, xt.shape), Tensor<float32, CUDA>(std::vector<int64>{ rows }),
 		Tensor<float32, CUDA>(std::vector<int64>{ rows }) };
@@ -74,6 +75,7 @@ inline LayerNormGradients<dtype> tensor_layer_norm_backward(const Tensor<dtype, 
 {
 	const int64 dim = xt.dim, d = xt.shape[dim - 1], rows = xt.numel() / d;
 	ACASSERT(dyt.dim == dim && dyt.numel() == xt.numel() && dyt.shape[dim - 1] == d, "dyt and xt need to have the same shape");
+	ACASSERT(b200_even_rows(xt, dim - 1) && b200_even_rows(dyt, dim - 1), "the rows need to be evenly spaced and dense");
 	ACASSERT(wt.shape[0] == d && mean.numel() == rows && rstd.numel() == rows, "wt, mean or rstd shape is incorrect");
 	LayerNormGradients<dtype> r{ Tensor<dtype, CUDA>(dim, xt.shape), Tensor<float32, CUDA>(std::vector<int64>{ d }),
 		Tensor<float32, CUDA>(std::vector<int64>{ d }) };

@@ -38,6 +38,14 @@ struct Step
 	void run() { tensor_selective_scan_update(state, x, dt, A, B, C); }
 };
 
+// 2 x 7 rows of 5 columns
+struct Norm
+{
+	T x = layout({ 2, 7, 5 }), dy = x, w = layout({ 5 }), b = w, mean = layout({ 14 }), rstd = mean;
+	void run() const { tensor_layer_norm(x, -1, w, b, 1e-5f); }
+	void gradient() const { tensor_layer_norm_backward(dy, x, w, mean, rstd); }
+};
+
 int main(int argc, char** argv)
 {
 	const std::map<std::string, std::function<void()>> cases = {
@@ -60,6 +68,15 @@ int main(int argc, char** argv)
 		{ "step B of sliced states", [] { Step s; s.B = layout({ 2, 2, 3 }, { 12, 6, 1 }); s.run(); } },
 		{ "step C of sliced states", [] { Step s; s.C = layout({ 2, 2, 3 }, { 12, 6, 1 }); s.run(); } },
 		{ "step channels apart", [] { Step s; s.dt = layout({ 2, 4 }, { 8, 2 }); s.run(); } },
+		{ "norm", [] { Norm().run(); } },
+		{ "norm gradient", [] { Norm().gradient(); } },
+		{ "norm of wider rows", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 7 * 9, 9, 1 }); s.run(); } },
+		{ "norm of one row", [] { Norm s; s.x = layout({ 5 }); s.run(); } },
+		// rows cut out of every matrix: the second matrix does not follow the first one's last row
+		{ "norm of cut rows", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 9 * 5, 5, 1 }); s.run(); } },
+		{ "norm columns apart", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 7 * 10, 10, 2 }); s.run(); } },
+		{ "norm gradient of cut rows", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 9 * 5, 5, 1 }); s.gradient(); } },
+		{ "norm gradient of cut dy", [] { Norm s; s.dy = layout({ 2, 7, 5 }, { 9 * 5, 5, 1 }); s.gradient(); } },
 	};
 	if (argc < 2 || !cases.count(argv[1])) return 2;
 	cases.at(argv[1])();

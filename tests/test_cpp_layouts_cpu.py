@@ -11,12 +11,14 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests", "cpp"))
 
 TAKEN = ["scan", "scan gradient", "scan rows of groups", "scan one group of wider rows", "scan channels of wider rows", "step", "step rows of groups",
-         "step one group of wider rows"]
+         "step one group of wider rows", "norm", "norm gradient", "norm of wider rows", "norm of one row"]
 REFUSED = {
     "scan B of sliced states": "not evenly spaced", "scan C of sliced states": "not evenly spaced",
     "scan gradient C of sliced states": "not evenly spaced", "scan B states apart": "not evenly spaced", "scan channels apart": "not evenly spaced",
     "scan gradient dy channels apart": "dy does not match x", "step B of sliced states": "rows are not dense", "step C of sliced states": "rows are not dense",
     "step channels apart": "rows are not dense",
+    "norm of cut rows": "evenly spaced", "norm columns apart": "evenly spaced", "norm gradient of cut rows": "evenly spaced",
+    "norm gradient of cut dy": "evenly spaced",
 }
 
 
