@@ -38,7 +38,7 @@ template <typename dtype>
 inline Tensor<dtype, CUDA> tensor_causal_conv1d_tokens(const Tensor<dtype, CUDA>& xt, const Tensor<dtype, CUDA>& wt, const Tensor<dtype, CUDA>& bt)
 {
 	ACASSERT(xt.dim == 3 && xt.shape[2] == wt.shape[0] && wt.shape[0] == bt.shape[0], "xt (batch, seq_len, dims), wt (dims, width), bt (dims)");
-	ACASSERT(xt.stride[0] == xt.shape[1] * xt.stride[1], "the rows of xt need to be evenly spaced");
+	ACASSERT(b200_even_rows(xt, 2) && b200_dense(wt, 0) && b200_dense(bt, 0), "the rows of xt need to be evenly spaced and dense, wt and bt dense");
 	Tensor<dtype, CUDA> yt(xt.dim, xt.shape);
 	b200_check(b200_causal_conv1d_tokens(b200_dtype_of<dtype>(), xt.buffer(), xt.stride[1], wt.buffer(), bt.buffer(), yt.buffer(), yt.stride[1],
 		nullptr, nullptr, xt.shape[0], xt.shape[1], xt.shape[2], static_cast<int>(wt.shape[1]), nullptr), "tensor_causal_conv1d_tokens");
@@ -60,7 +60,8 @@ inline CausalConv1dGradients<dtype> tensor_causal_conv1d_tokens_backward(const T
 {
 	ACASSERT(xt.dim == 3 && xt.shape[2] == wt.shape[0] && wt.shape[0] == bt.shape[0], "xt (batch, seq_len, dims), wt (dims, width), bt (dims)");
 	ACASSERT(dyt.dim == 3 && dyt.shape[0] == xt.shape[0] && dyt.shape[1] == xt.shape[1] && dyt.shape[2] == xt.shape[2], "dyt and xt need to have the same shape");
-	ACASSERT(xt.stride[0] == xt.shape[1] * xt.stride[1] && dyt.stride[0] == dyt.shape[1] * dyt.stride[1], "the rows need to be evenly spaced");
+	ACASSERT(b200_even_rows(xt, 2) && b200_even_rows(dyt, 2) && b200_dense(wt, 0) && b200_dense(bt, 0),
+		"the rows need to be evenly spaced and dense, wt and bt dense");
 	const int64 b = xt.shape[0], l = xt.shape[1], d = xt.shape[2];
 	const int width = static_cast<int>(wt.shape[1]);
 	CausalConv1dGradients<dtype> r{ Tensor<dtype, CUDA>(xt.dim, xt.shape), Tensor<float32, CUDA>(std::vector<int64>{ d, width }),

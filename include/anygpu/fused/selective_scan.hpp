@@ -29,6 +29,8 @@ struct SelectiveScanArgs
 		ACASSERT(dt.shape[2] == d && (!z || (z->dim == 3 && z->shape[2] == d)), "dt or z does not match x");
 		ACASSERT((!D || D->numel() == d) && (!dt_bias || dt_bias->numel() == d), "D or dt_bias does not match x");
 		ACASSERT(!initial_states || initial_states->numel() == b * d * n, "initial_states does not match");
+		ACASSERT(b200_dense(A, 0) && (!D || b200_dense(*D, 0)) && (!dt_bias || b200_dense(*dt_bias, 0)) && (!initial_states || b200_dense(*initial_states, 0)),
+			"A, D, dt_bias and initial_states need to be dense");
 		return { x.buffer(), dt.buffer(), B.buffer(), C.buffer(), z ? z->buffer() : nullptr, x.stride[1], dt.stride[1], B.stride[1], C.stride[1],
 			z ? z->stride[1] : 0, A.buffer(), D ? D->buffer() : nullptr, dt_bias ? dt_bias->buffer() : nullptr,
 			initial_states ? initial_states->buffer() : nullptr, 0, 1, b, l, d, g, n };
@@ -76,6 +78,8 @@ inline Tensor<dtype, CUDA> tensor_selective_scan_update(Tensor<float32, CUDA>& s
 	ACASSERT((!z || (z->dim == 2 && z->shape[0] == b && z->shape[1] == d)) && (!D || D->numel() == d) && (!dt_bias || dt_bias->numel() == d),
 		"z, D or dt_bias does not match x");
 	ACASSERT(b200_dense(x, 1) && b200_dense(dt, 1) && b200_dense(B, 1) && b200_dense(C, 1) && (!z || b200_dense(*z, 1)), "rows are not dense");
+	ACASSERT(b200_dense(state, 0) && b200_dense(A, 0) && (!D || b200_dense(*D, 0)) && (!dt_bias || b200_dense(*dt_bias, 0)),
+		"state, A, D and dt_bias need to be dense");
 	Tensor<dtype, CUDA> y(x.dim, x.shape);
 	b200_check(b200_selective_scan_update(b200_dtype_of<dtype>(), state.buffer(), x.buffer(), x.stride[0], dt.buffer(), dt.stride[0], A.buffer(), 0,
 		B.buffer(), B.stride[0], C.buffer(), C.stride[0], D ? D->buffer() : nullptr, dt_bias ? dt_bias->buffer() : nullptr, z ? z->buffer() : nullptr,
@@ -100,7 +104,8 @@ inline SelectiveScanGradients<dtype> tensor_selective_scan_backward(const Tensor
 		b200_dense(dy, 2), "dy does not match x");
 	ACASSERT(static_cast<size_t>(checkpoints.numel()) * sizeof(float) == b200_selective_scan_checkpoint_bytes(in.batch, in.seqlen, in.dim, in.d_state),
 		"checkpoints are not of this call");
-	ACASSERT(!dfinal_states || dfinal_states->numel() == in.batch * in.dim * in.d_state, "dfinal_states does not match");
+	ACASSERT(b200_dense(checkpoints, 0) && (!dfinal_states || (dfinal_states->numel() == in.batch * in.dim * in.d_state && b200_dense(*dfinal_states, 0))),
+		"dfinal_states does not match, or it or checkpoints is not dense");
 	SelectiveScanGradients<dtype> r;
 	r.dx = Tensor<dtype, CUDA>(args.x.dim, args.x.shape);
 	r.ddt = Tensor<dtype, CUDA>(args.x.dim, args.x.shape);

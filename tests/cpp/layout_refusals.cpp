@@ -46,6 +46,14 @@ struct Norm
 	void gradient() const { tensor_layer_norm_backward(dy, x, w, mean, rstd); }
 };
 
+// 2 x 7 tokens of 5 channels, width 4
+struct Conv
+{
+	T x = layout({ 2, 7, 5 }), dy = x, w = layout({ 5, 4 }), b = layout({ 5 });
+	void run() const { tensor_causal_conv1d_tokens(x, w, b); }
+	void gradient() const { tensor_causal_conv1d_tokens_backward(dy, x, w, b); }
+};
+
 int main(int argc, char** argv)
 {
 	const std::map<std::string, std::function<void()>> cases = {
@@ -77,6 +85,21 @@ int main(int argc, char** argv)
 		{ "norm columns apart", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 7 * 10, 10, 2 }); s.run(); } },
 		{ "norm gradient of cut rows", [] { Norm s; s.x = layout({ 2, 7, 5 }, { 9 * 5, 5, 1 }); s.gradient(); } },
 		{ "norm gradient of cut dy", [] { Norm s; s.dy = layout({ 2, 7, 5 }, { 9 * 5, 5, 1 }); s.gradient(); } },
+		{ "conv", [] { Conv().run(); } },
+		{ "conv gradient", [] { Conv().gradient(); } },
+		{ "conv of wider rows", [] { Conv s; s.x = layout({ 2, 7, 5 }, { 7 * 9, 9, 1 }); s.run(); } },
+		// parameters and states have no stride of their own in the C ABI: slices of wider ones are not where the kernels look
+		{ "conv sliced w", [] { Conv s; s.w = layout({ 5, 4 }, { 8, 1 }); s.run(); } },
+		{ "conv channels apart", [] { Conv s; s.x = layout({ 2, 7, 5 }, { 7 * 10, 10, 2 }); s.run(); } },
+		{ "conv gradient sliced w", [] { Conv s; s.w = layout({ 5, 4 }, { 8, 1 }); s.gradient(); } },
+		{ "conv gradient channels apart", [] { Conv s; s.dy = layout({ 2, 7, 5 }, { 7 * 10, 10, 2 }); s.gradient(); } },
+		{ "scan sliced A", [] { Scan s; s.A = layout({ 4, 3 }, { 6, 1 }); s.run(); } },
+		{ "scan sliced initial states", [] { Scan s; T i = layout({ 2, 4, 3 }, { 24, 6, 1 });
+			tensor_selective_scan(SelectiveScanArgs<float32>{ s.x, s.dt, s.A, s.B, s.C, nullptr, nullptr, nullptr, &i }); } },
+		{ "scan gradient sliced dfinal states", [] { Scan s; T f = layout({ 2, 4, 3 }, { 24, 6, 1 });
+			tensor_selective_scan_backward(s.dy, s.args(), s.ck, &f); } },
+		{ "step sliced A", [] { Step s; s.A = layout({ 4, 3 }, { 6, 1 }); s.run(); } },
+		{ "step sliced state", [] { Step s; s.state = layout({ 2, 4, 3 }, { 24, 6, 1 }); s.run(); } },
 	};
 	if (argc < 2 || !cases.count(argv[1])) return 2;
 	cases.at(argv[1])();

@@ -11,7 +11,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "tests", "cpp"))
 
 TAKEN = ["scan", "scan gradient", "scan rows of groups", "scan one group of wider rows", "scan channels of wider rows", "step", "step rows of groups",
-         "step one group of wider rows", "norm", "norm gradient", "norm of wider rows", "norm of one row"]
+         "step one group of wider rows", "norm", "norm gradient", "norm of wider rows", "norm of one row",
+         "conv", "conv gradient", "conv of wider rows"]
 REFUSED = {
     "scan B of sliced states": "not evenly spaced", "scan C of sliced states": "not evenly spaced",
     "scan gradient C of sliced states": "not evenly spaced", "scan B states apart": "not evenly spaced", "scan channels apart": "not evenly spaced",
@@ -19,6 +20,9 @@ REFUSED = {
     "step channels apart": "rows are not dense",
     "norm of cut rows": "evenly spaced", "norm columns apart": "evenly spaced", "norm gradient of cut rows": "evenly spaced",
     "norm gradient of cut dy": "evenly spaced",
+    "conv sliced w": "dense", "conv channels apart": "dense", "conv gradient sliced w": "dense", "conv gradient channels apart": "dense",
+    "scan sliced A": "dense", "scan sliced initial states": "dense", "scan gradient sliced dfinal states": "dense", "step sliced A": "dense",
+    "step sliced state": "dense",
 }
 
 
