@@ -75,7 +75,13 @@ def _check(t, name, shape, dtype, contiguous=False):
 
 
 def _param(t, name, shape):
-    """An optional fp32 parameter or state: contiguous, 16-byte aligned."""
+    """An optional fp32 parameter: contiguous, on any element."""
+    if t is not None:
+        _check(t, name, shape, torch.float32, contiguous=True)
+
+
+def _state(t, name, shape):
+    """An optional fp32 state: contiguous, 16-byte aligned."""
     if t is not None:
         _check(t, name, shape, torch.float32, contiguous=True)
         assert t.data_ptr() % 16 == 0, f"{name} must start on a 16-byte boundary"
@@ -324,8 +330,8 @@ def tensor_selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_
     assert x.dim() == 3
     b, l, d = x.shape
     g, n = _scan_shapes(x, dt, A, B, C, D, z, dt_bias)
-    _param(initial_states, "initial_states", (b, d, n))
-    _param(final_states_out, "final_states_out", (b, d, n))
+    _state(initial_states, "initial_states", (b, d, n))
+    _state(final_states_out, "final_states_out", (b, d, n))
     with _on_device(x, dt, A, B, C, D, z, dt_bias, initial_states, final_states_out):
         lib = capi.load()
         inp = _scan_inputs(x, dt, A, B, C, D, z, dt_bias, initial_states, a_is_log, dt_softplus, g, n)
@@ -346,7 +352,7 @@ def tensor_selective_scan_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=
     assert x.dim() == 2
     b, d = x.shape
     g, n = _scan_shapes(x, dt, A, B, C, D, z, dt_bias)
-    _param(state, "state", (b, d, n))
+    _state(state, "state", (b, d, n))
     with _on_device(state, x, dt, A, B, C, D, z, dt_bias):
         y = x.new_empty((b, d))
         capi.call("b200_selective_scan_update", _dt(x), _ptr(state), _ptr(x), _row_stride(x, "x", d), _ptr(dt), _row_stride(dt, "dt", d), _ptr(A),
@@ -377,10 +383,10 @@ def tensor_selective_scan_backward(dy, x, dt, A, B, C, checkpoints, D=None, z=No
     b, l, d = x.shape
     g, n = _scan_shapes(x, dt, A, B, C, D, z, dt_bias)
     _check(dy, "dy", x.shape, x.dtype)
-    _param(initial_states, "initial_states", (b, d, n))
-    _param(dfinal_states, "dfinal_states", (b, d, n))
+    _state(initial_states, "initial_states", (b, d, n))
+    _state(dfinal_states, "dfinal_states", (b, d, n))
     lib = capi.load()
-    _param(checkpoints, "checkpoints", (lib.b200_selective_scan_checkpoint_bytes(b, l, d, n) // 4,))
+    _state(checkpoints, "checkpoints", (lib.b200_selective_scan_checkpoint_bytes(b, l, d, n) // 4,))
     with _on_device(dy, x, dt, A, B, C, checkpoints, D, z, dt_bias, initial_states, dfinal_states):
         inp = _scan_inputs(x, dt, A, B, C, D, z, dt_bias, initial_states, a_is_log, dt_softplus, g, n)
         act = lambda *shape: x.new_empty(shape)
