@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kForwardThreads, 2) selective_scan_kernel(cons
 			{
 				float zv[EPT], sg[EPT];
 				raw_read<T, EPT>(slot(3, buf), zv, lane);
-				sigmoid_n<EPT>(zv, sg);
+				sigmoid_n<EPT, EXACT>(zv, sg);
 #pragma unroll
 				for (int e = 0; e < EPT; ++e) o[e] *= zv[e] * sg[e];
 			}
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(128) selective_scan_update_kernel(float* __res
 #pragma unroll
 	for (int r = 0; r < RB; ++r) dv[r] += bias;
 	if (in.softplus) softplus_n<RB>(dv);
-	sigmoid_n<RB>(zv, sg);
+	sigmoid_n<RB, sizeof(T) == 4>(zv, sg);
 #pragma unroll
 	for (int r = 0; r < RB; ++r)
 	{

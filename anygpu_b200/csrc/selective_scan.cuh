@@ -10,6 +10,7 @@ constexpr int kTok = 16;      // tokens between two saved states, from which the
 constexpr int kMaxState = 32 * kStates;
 constexpr int kMaxWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e));  // log2(e) = kLog2e + kLog2eLow
 
 // Lanes that share a channel of n states: the smallest power of two whose lanes hold them all.
 inline int lanes_per_channel(int64_t n)
@@ -45,22 +46,12 @@ __device__ __forceinline__ f2 exp2_2(f2 a)
 	const float2 v = unpack2(a);
 	return pack2(exp2_approx(v.x), exp2_approx(v.y));
 }
-// 2^x of a pair to half a step of fp32, without the exponential unit: x = n + f, n the nearest integer (added and taken away with
-// 1.5 * 2^23, which leaves n in the low bits), f in [-1/2, 1/2]; 2^f by its minimax polynomial of degree 6 with constant term 1
-// (relative error 2^-28.9, and exact at 0, where the decays of slow states lie), times the float whose exponent field is n + 127. (An
-// integer addition of n to the polynomial's exponent would save that multiplication, but turns NaN into a number.) Below x = -126.5 that
-// field is 0 and the result zero: a decay that forgets the state leaves nothing of it for A, which may be as large as floats go, to
-// magnify in the gradients. From x = 127.5 on the result is infinite, NaN stays NaN.
-__device__ __forceinline__ f2 exp2_poly_2(f2 x)
+// 2^(n + f) of a pair: f in [-1/2, 1/2] up to rounding, t = 1.5 * 2^23 + n, which holds the integer n in its low bits. 2^f by its minimax
+// polynomial of degree 6 with constant term 1 (relative error 2^-28.9, and exact at 0, where the decays of slow states lie), times the
+// float whose exponent field is n + 127, n in [-127, 128]. (An integer addition of n to the polynomial's exponent would save that
+// multiplication, but turns NaN into a number.)
+__device__ __forceinline__ f2 pow2_split(f2 t, f2 f)
 {
-	float2 v = unpack2(x);
-	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.f));
-	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.f));
-	asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(128.f));
-	asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(128.f));
-	const f2 c = pack2(v.x, v.y);
-	const f2 t = add2(c, both(12582912.f));
-	const f2 f = add2(c, fma2(t, both(-1.f), both(12582912.f)));
 	f2 p = both(1.535336179e-04f);
 	p = fma2(p, f, both(1.339887446e-03f));
 	p = fma2(p, f, both(9.618437358e-03f));
@@ -70,6 +61,41 @@ __device__ __forceinline__ f2 exp2_poly_2(f2 x)
 	p = fma2(p, f, both(1.f));
 	const float2 n = unpack2(t);
 	return mul2(p, pack2(__int_as_float((__float_as_int(n.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
+}
+// NaN stays NaN.
+template <bool LOW_ONLY = false>
+__device__ __forceinline__ f2 clamp_2(f2 x, float lo, float hi)
+{
+	float2 v = unpack2(x);
+	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(lo));
+	asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(lo));
+	if constexpr (!LOW_ONLY)
+	{
+		asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(hi));
+		asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(hi));
+	}
+	return pack2(v.x, v.y);
+}
+// 2^x of a pair to half a step of fp32, without the exponential unit: x = n + f, n the nearest integer (added and taken away with
+// 1.5 * 2^23). Below x = -126.5 the exponent field is 0 and the result zero: a decay that forgets the state leaves nothing of it for A,
+// which may be as large as floats go, to magnify in the gradients. From x = 127.5 on the result is infinite, NaN stays NaN.
+__device__ __forceinline__ f2 exp2_poly_2(f2 x)
+{
+	const f2 c = clamp_2(x, -127.f, 128.f);
+	const f2 t = add2(c, both(12582912.f));
+	return pow2_split(t, add2(c, fma2(t, both(-1.f), both(12582912.f))));
+}
+// e^v of a pair to two half steps (2^-24) of fp32. v log2(e) rounded once would be off by |v| half steps of the result; here the integer part is taken
+// from it and the fraction is v log2(e) - n in multiply-adds, which round once, with log2(e) in two floats. Zero below v = -87.7, infinite from
+// 88.4 on, NaN stays NaN.
+template <bool NEGATIVE = false /* v <= 0 */>
+__device__ __forceinline__ f2 exp_2(f2 v)
+{
+	const f2 c = clamp_2<NEGATIVE>(v, -88.1f, 88.6f);  // times log2(e): -127.1, 127.8
+	const f2 t = fma2(c, both(kLog2e), both(12582912.f));
+	f2 f = fma2(c, both(kLog2e), fma2(t, both(-1.f), both(12582912.f)));
+	f = fma2(c, both(kLog2eLow), f);
+	return pow2_split(t, f);
 }
 // The decays of one token. The exponential unit's 2^-22 adds up over a long memory: with it everywhere dA is off by 1.9e-6 and
 // final_state by 4.8e-7 (8192 x 4096 x 16, f16 activations), with the polynomial everywhere by 3.4e-7 and 1.4e-7, at 396 instead of 228 us
@@ -100,7 +126,7 @@ __device__ __forceinline__ f2 rcp_2(f2 a)
 __device__ __forceinline__ f2 softplus_2(f2 v)
 {
 	const float2 a = unpack2(v);
-	const f2 w = exp2_2(mul2(pack2(fabsf(a.x), fabsf(a.y)), both(-kLog2e)));
+	const f2 w = exp_2<true>(pack2(-fabsf(a.x), -fabsf(a.y)));
 	const f2 s = mul2(w, rcp_2(add2(w, both(2.f))));
 	const f2 q = mul2(s, s);
 	f2 p = both(2.f / 13.f);
@@ -112,8 +138,16 @@ __device__ __forceinline__ f2 softplus_2(f2 v)
 	p = fma2(p, q, both(2.f));
 	return fma2(p, s, pack2(a.x > 0.f ? a.x : 0.f, a.y > 0.f ? a.y : 0.f));
 }
-// 1 / (1 + exp(-v))
-__device__ __forceinline__ f2 sigmoid_2(f2 v) { return rcp_2(add2(exp2_2(mul2(v, both(-kLog2e))), both(1.f))); }
+// 1 / (1 + exp(-v)). EXACT (fp32 calls, and softplus' everywhere, which ddt_bias sums in fp32): e^-v to two half steps. Else through the exponential
+// unit, off by |v| half steps for the rounding of v log2(e): the gate of f16 calls, whose results are rounded by 2^13 of them. (With it everywhere
+// the step sizes were off by 1.7e-7 rms instead of 6.8e-8 and those at v = -60 by 56 u. It costs the f16 training step of 4 x 2048 x 4096 x 16 1250 ->
+// 1275 us, the prompt 228 -> 230; with the gates too 1304 and 231. fp32: prompt 438 -> 429, training step of 4 x 1024 835 -> 860.)
+template <bool EXACT>
+__device__ __forceinline__ f2 sigmoid_2(f2 v)
+{
+	const f2 e = EXACT ? exp_2(mul2(v, both(-1.f))) : exp2_2(mul2(v, both(-kLog2e)));
+	return rcp_2(add2(e, both(1.f)));
+}
 // The same functions over an even or odd number of values.
 template <int E>
 __device__ __forceinline__ void softplus_n(float* v)
@@ -126,13 +160,13 @@ __device__ __forceinline__ void softplus_n(float* v)
 		if (e + 1 < E) v[e + 1] = r.y;
 	}
 }
-template <int E>
+template <int E, bool EXACT>
 __device__ __forceinline__ void sigmoid_n(const float* v, float* o)
 {
 #pragma unroll
 	for (int e = 0; e < E; e += 2)
 	{
-		const float2 r = unpack2(sigmoid_2(pack2(v[e], v[e + 1 < E ? e + 1 : e])));
+		const float2 r = unpack2(sigmoid_2<EXACT>(pack2(v[e], v[e + 1 < E ? e + 1 : e])));
 		o[e] = r.x;
 		if (e + 1 < E) o[e + 1] = r.y;
 	}

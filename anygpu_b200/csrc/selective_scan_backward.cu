@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 			{
 				float zv[EPT], sg[EPT];
 				raw_read<T, EPT>(raw + 2 * RAW1, zv, lane);
-				sigmoid_n<EPT>(zv, sg);
+				sigmoid_n<EPT, sizeof(T) == 4>(zv, sg);
 #pragma unroll
 				for (int e = 0; e < EPT; ++e) gv[e] *= zv[e] * sg[e];
 			}
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 				{
 					float sg[EPT];
 					raw_read<T, EPT>(raw + 2 * RAW1, zv, lane);
-					sigmoid_n<EPT>(zv, sg);
+					sigmoid_n<EPT, sizeof(T) == 4>(zv, sg);
 #pragma unroll
 					for (int e = 0; e < EPT; ++e)
 					{
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 					for (int e = 0; e < EPT; ++e) ds[e] = gv[e];
 #pragma unroll
 				for (int e = 0; e < EPT; ++e) dv[e] += t_bias[e];
-				if (in.softplus) sigmoid_n<EPT>(dv, dv);
+				if (in.softplus) sigmoid_n<EPT, true>(dv, dv);
 #pragma unroll
 				for (int e = 0; e < EPT; ++e)
 				{
