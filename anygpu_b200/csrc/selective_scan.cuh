@@ -329,14 +329,15 @@ struct RowsBC
 	__device__ __forceinline__ RowsBC(int tid_, int threads_) : tid(tid_), threads(threads_) {}
 
 
-	static __device__ __forceinline__ const T* at(const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end, int k)
+	// pad: empty places at the head of the tile
+	static __device__ __forceinline__ const T* at(const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end, int k, int pad = 0)
 	{
 		const int n = k % NP, tt = (k / NP) % TT;
 		const int64_t t = t0 + tt;
-		if (t >= t_end || n >= in.N) return nullptr;
+		if (t >= t_end || n >= in.N || tt < pad) return nullptr;
 		return k < TT * NP ? B + t * in.Bs + n : C + t * in.Cs + n;
 	}
-	__device__ __forceinline__ void fetch(bool vec, const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end)
+	__device__ __forceinline__ void fetch(bool vec, const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end, int pad = 0)
 	{
 		if (!vec) return;
 #pragma unroll
@@ -346,7 +347,7 @@ struct RowsBC
 			pre[i] = make_uint4(0, 0, 0, 0);
 			if (k < TOTAL)
 			{
-				const T* p = at(in, B, C, t0, t_end, k);
+				const T* p = at(in, B, C, t0, t_end, k, pad);
 				if (p) pre[i] = *reinterpret_cast<const uint4*>(p);
 			}
 		}
@@ -389,7 +390,7 @@ struct RowsBC
 	// The same into ORDERS copies of the tile whose groups of four states are permuted: copy p * ORDERS / 4 holds state i ^ p of a group in
 	// place i (p = 0, 2 for two orders).
 	template <int ORDERS, int COPY /* elements from copy to copy */>
-	__device__ __forceinline__ void store_orders(bool vec, const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end, float* s)
+	__device__ __forceinline__ void store_orders(bool vec, const Inputs& in, const T* B, const T* C, int64_t t0, int64_t t_end, int pad, float* s)
 	{
 		auto put_orders = [&](int k, float4 v) {
 #pragma unroll
@@ -416,7 +417,7 @@ struct RowsBC
 			}
 			for (int k = (tid + PRE * threads) * EB; k < TOTAL; k += threads * EB)
 			{
-				const T* p = at(in, B, C, t0, t_end, k);
+				const T* p = at(in, B, C, t0, t_end, k, pad);
 				uint4 v = make_uint4(0, 0, 0, 0);
 				if (p) v = *reinterpret_cast<const uint4*>(p);
 				put_vec(k, v);
@@ -430,7 +431,7 @@ struct RowsBC
 #pragma unroll
 				for (int j = 0; j < 4; ++j)
 				{
-					const T* p = at(in, B, C, t0, t_end, k + j);
+					const T* p = at(in, B, C, t0, t_end, k + j, pad);
 					v[j] = p ? Cvt<T>::to_f32(*p) : 0.f;
 				}
 				put_orders(k, make_float4(v[0], v[1], v[2], v[3]));

@@ -243,9 +243,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 	const bool vec_bc = in.vec_bc;
 	float hn[kStates] = { 0.f, 0.f, 0.f, 0.f };  // the state before the next tile
 	const int64_t nk = cdiv(in.seqlen, kTok);
-	auto fetch = [&](int64_t t0, int buf) {
-		const int64_t t = t0 + lt;
-		const int n = t < t_end ? cn : 0;
+	auto fetch = [&](int64_t t0, int buf, int pad) {
+		const int64_t t = t0 + lt - pad;
+		const int n = lt >= pad ? cn : 0;
 		const int64_t tc = n > 0 ? t : t_begin;  // an address inside the tensor even where nothing is read
 		unsigned char* r = s_raw + buf * 4 * RAW1;
 		if (MODE == 0) raw_load<T, EPT, VEC>(r, xp + tc * in.xs, n, lane);
@@ -253,16 +253,16 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 		if (zp) raw_load<T, EPT, VEC>(r + 2 * RAW1, zp + tc * in.zs, n, lane);
 		raw_load<T, EPT, VEC>(r + 3 * RAW1, yp + tc * ar.dys, n, lane);
 		asm volatile("cp.async.commit_group;" ::: "memory");
-		bc.fetch(vec_bc, in, Bp, Cp, t0, t_end);
+		bc.fetch(vec_bc, in, Bp, Cp, t0 - pad, t_end, pad);
 		if (MODE == 0 && mine) load_states(vec4, hn, ar.ckpt + ((b * nk + t0 / kTok) * in.dim + c) * N, n0, N);
 	};
 	// dB and dC of a finished tile: the warps in order, one partial row per CTA
-	auto join_warps = [&](int64_t t0) {
-		float* pr = ar.part_BC + (static_cast<int64_t>(blockIdx.x) * gridDim.y * in.seqlen + tok0 + t0) * 2 * N;
+	auto join_warps = [&](int64_t t0, int pad) {
+		float* pr = ar.part_BC + (static_cast<int64_t>(blockIdx.x) * gridDim.y * in.seqlen + tok0 + t0 - pad) * 2 * N;
 		for (int k = threadIdx.x * 4; k < kTok * ROW; k += blockDim.x * 4)
 		{
 			const int n = k % NP, t = k / ROW;
-			if (n >= N || t0 + t >= t_end) continue;
+			if (n >= N || t < pad) continue;
 			const unsigned char* r = smem + AT_RED + k * 4;  // of warp 0
 			f2 s[2] = { 0ull, 0ull };
 #pragma unroll
@@ -277,13 +277,16 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 		}
 	};
 
+	// A last tile that is not full has its empty places at the head (place lt is token t0 + lt - pad): the walk backwards meets its tokens
+	// first, and what the empty places, whose steps are zero, make of NaN in A (exp(0 A)) comes after a token that did the same.
 	const int64_t last = t_begin + (t_end - 1 - t_begin) / kTok * kTok;
-	fetch(last, 0);
+	int pad = static_cast<int>(last + kTok - t_end);
+	fetch(last, 0, pad);
 	int buf = 0;
-	for (int64_t t0 = last; t0 >= t_begin; t0 -= kTok, buf ^= 1)
+	for (int64_t t0 = last; t0 >= t_begin; t0 -= kTok, buf ^= 1, pad = 0)
 	{
 		const unsigned char* raw = s_raw + buf * 4 * RAW1;
-		const bool tok = loads && t0 + lt < t_end;
+		const bool tok = loads && lt >= pad;
 		asm volatile("cp.async.wait_group 0;" ::: "memory");
 		if (loads)
 		{
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 				t_ds[e * DS] = both(gv[e]);
 			}
 		}
-		bc.template store_orders<S::ORDERS, M::BC / 4>(vec_bc, in, Bp, Cp, t0, t_end, s_bc);
+		bc.template store_orders<S::ORDERS, M::BC / 4>(vec_bc, in, Bp, Cp, t0 - pad, t_end, pad, s_bc);
 		const float* s_B = s_bc + (ord * S::ORDERS / 4) * (M::BC / 4);
 		const float* s_C = s_B + kTok * NP;
 		f2 hb[2];  // the state before this tile
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 		hb[0] = pack2(hn[0], hn[1]);
 		hb[1] = pack2(hn[2], hn[3]);
 		__syncthreads();
-		if (t0 > t_begin) fetch(t0 - kTok, buf ^ 1);
+		if (t0 > t_begin) fetch(t0 - kTok, buf ^ 1, 0);
 		const ulonglong2* pp = reinterpret_cast<const ulonglong2*>(own) + cl * PS;
 		const f2* pd = reinterpret_cast<const f2*>(own + AT_DS) + cl * DS;
 		if constexpr (MODE == 1)
@@ -418,10 +421,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) selective_scan_backward_ker
 			aA[0] = add2(aA[0], tile_A[0]);
 			aA[1] = add2(aA[1], tile_A[1]);
 			__syncthreads();
-			if (ar.part_BC) join_warps(t0);
+			if (ar.part_BC) join_warps(t0, pad);
 			if (tok)
 			{
-				const int64_t t = tok0 + t0 + lt;
+				const int64_t t = tok0 + t0 + lt - pad;
 				float xv[EPT], dv[EPT], gv[EPT], zv[EPT], ox[EPT], od[EPT], ds[EPT];
 				raw_read<T, EPT>(raw, xv, lane);
 				raw_read<T, EPT>(raw + RAW1, dv, lane);

@@ -104,3 +104,24 @@ def test_masked_tokens_of_channels_that_forget(ops, shape, dtype, mask):
                 ref.assert_within(getattr(grads, name)[i:i + 1, kept], leaves[leaf].grad, bounds[2 + j], name)
             elif leaf == "init":
                 ref.assert_within(grads.dinitial_states[i:i + 1], leaves[leaf].grad, bounds[2 + j], name)
+
+
+@pytest.mark.parametrize("shape", [(2, 40, 20, 1, 16), (1, 33, 12, 2, 5), (1, 31, 9, 1, 3), (2, 17, 8, 1, 100), (1, 3, 16, 1, 16), (1, 700, 8, 1, 16)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("log", [False, True])
+def test_a_decay_that_is_not_a_number_reaches_what_it_should(ops, shape, dtype, log):
+    """NaN in one element of A, sequences that end inside a tile: results and gradients are NaN exactly where the 64-bit form's are, the last
+    token's (which no decay separates from the final state) among them."""
+    b, l, d, g, n = shape
+    p, gen = inputs(l + d, b, l, d, g, n, dtype, log=log)
+    p["A"][5, 2] = float("nan")
+    dy, dfin = rn(gen, b, l, d, dtype=dtype), rn(gen, b, d, n)
+    y, fin, ck = ops.tensor_selective_scan(**p, a_is_log=log, want_checkpoints=True)
+    grads = ops.tensor_selective_scan_backward(dy, checkpoints=ck, dfinal_states=dfin, **p, a_is_log=log)
+    leaves = {k: v.requires_grad_() for k, v in reference_args(p).items()}
+    wy, wfin = ref.scan(**leaves, log=log)
+    ((wy * dy.double()).sum() + (wfin * dfin.double()).sum()).backward()
+    assert not torch.isnan(leaves["x"].grad[:, -1]).any() and not torch.isnan(leaves["B"].grad[:, -1]).any()
+    for name, got, want in [("y", y, wy), ("final_states", fin, wfin)] + [(name, getattr(grads, name), leaves[leaf].grad) for name, leaf in GRADS]:
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{name}: {int(torch.isnan(got).sum())} against {int(torch.isnan(want).sum())}"
+        assert torch.isfinite(got[~torch.isnan(got)]).all(), name
