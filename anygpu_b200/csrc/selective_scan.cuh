@@ -184,26 +184,11 @@ struct alignas(16) Frag
 enum Access { kSingle, kWords, kVectors };
 
 // Missing channels read zero and are not written.
-template <typename T, int EPT, Access VEC>
+template <typename T, int EPT>
 __device__ __forceinline__ void load_frag(Frag<T, EPT>& f, const T* p, int n)
 {
-	if constexpr (VEC == kVectors)
-	{
-		constexpr int BYTES = EPT * sizeof(T) < 16 ? EPT * sizeof(T) : 16;
-		using B = typename BitsOf<BYTES>::type;
 #pragma unroll
-		for (int i = 0; i < EPT * (int)sizeof(T) / BYTES; ++i)
-		{
-			B bits = {};
-			if (n > 0) bits = reinterpret_cast<const B*>(p)[i];
-			reinterpret_cast<B*>(f.v)[i] = bits;
-		}
-	}
-	else
-	{
-#pragma unroll
-		for (int e = 0; e < EPT; ++e) f.v[e] = e < n ? p[e] : Cvt<T>::from_f32(0.f);
-	}
+	for (int e = 0; e < EPT; ++e) f.v[e] = e < n ? p[e] : Cvt<T>::from_f32(0.f);
 }
 template <typename T, int EPT, Access VEC>
 __device__ __forceinline__ void store_frag(const float* o, T* p, int n)
@@ -253,7 +238,7 @@ __device__ __forceinline__ void frag_f32(const Frag<T, EPT>& f, float* o)
 		for (int e = 0; e < EPT; ++e) o[e] = Cvt<T>::to_f32(f.v[e]);
 	}
 }
-// Whether a tensor's rows can be read with load_frag's vectors: EPT channels per lane from channel offsets that are multiples of EPT.
+// Whether a tensor's rows allow kVectors: EPT channels at a time from channel offsets that are multiples of EPT.
 template <typename T, int EPT>
 inline bool frag_aligned(const void* p, int64_t stride)
 {
@@ -297,7 +282,7 @@ __device__ __forceinline__ void raw_load(unsigned char* s, const T* p, int n, in
 	else
 	{
 		Frag<T, EPT> f;
-		load_frag<T, EPT, kSingle>(f, p, n);
+		load_frag(f, p, n);
 		constexpr int PER = CH / sizeof(T);
 #pragma unroll
 		for (int e = 0; e < EPT; ++e) *reinterpret_cast<T*>(s + ((e / PER) * 32 + lane) * CH + (e % PER) * sizeof(T)) = f.v[e];
