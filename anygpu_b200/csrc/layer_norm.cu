@@ -552,16 +552,16 @@ __global__ void __launch_bounds__(256) layer_norm_dw_wide_kernel(const T* __rest
 constexpr int kRingBytes = 104 * 1024;   // of a CTA, two of which share an SM
 constexpr int kRingMax = 200 * 1024;     // of a CTA that has the SM for itself
 
-// Ring of stages of `unit` bytes each: stages and CTAs per SM; 0 stages: no ring (rows too long or too short).
+// Ring of stages of `unit` bytes each, 64 KB at most (two rows of 8192 fp32 columns, the longest that take it): stages and CTAs per SM.
 struct Ring
 {
 	int stages, ctas;
 };
 static Ring ring_of(int64_t unit)
 {
+	static_assert(kRingMax >= 2 * 65536, "two stages at least");
 	if (2 * unit <= kRingBytes) return { static_cast<int>(kRingBytes / unit < 4 ? kRingBytes / unit : 4), 2 };
-	if (2 * unit <= kRingMax) return { static_cast<int>(kRingMax / unit < 4 ? kRingMax / unit : 4), 1 };
-	return { 0, 0 };
+	return { static_cast<int>(kRingMax / unit < 4 ? kRingMax / unit : 4), 1 };
 }
 
 // partial rows of dw / db: the workspace holds the larger of what the two forms of the kernel want (a function of the sizes alone)
@@ -671,8 +671,9 @@ static int layer_norm_backward_v(const LnPlan& p, const T* dy, int64_t dys, cons
 {
 	if constexpr (V > 1)  // aligned rows that are not short take the ring: one warp, or two (f16)
 	{
-		if (p.threads == 32) return launch_ln_backward<T, V, 32>(p, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, st);
-		return launch_ln_backward<T, V, 64>(p, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, st);
+		if constexpr (sizeof(T) == 2)
+			if (p.threads == 64) return launch_ln_backward<T, V, 64>(p, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, st);
+		return launch_ln_backward<T, V, 32>(p, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, st);
 	}
 	else return with_ln_threads<false>(p.threads, [&](auto threads) {
 		return launch_ln_backward<T, V, decltype(threads)::value>(p, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, st);
@@ -730,7 +731,9 @@ static int layer_norm_backward(const void* dyv, int64_t dys, const void* xv, int
 			const int nv = static_cast<int>(cdiv(dim, static_cast<int64_t>(kRowThreads) * E));
 #define B200_LN_ROWS(NV, R) launch_ln_rows_backward<T, NV, R>(rp, dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, d, p.dimp, st)
 			if (rp.r == 2) rc = nv == 1 ? B200_LN_ROWS(1, 2) : B200_LN_ROWS(2, 2);
-			else rc = nv <= 3 ? B200_LN_ROWS(3, 1) : (nv <= 4 ? B200_LN_ROWS(4, 1) : B200_LN_ROWS(8, 1));
+			else if (nv <= 3) rc = B200_LN_ROWS(3, 1);
+			else if (sizeof(T) == 2 || nv == 4) rc = B200_LN_ROWS(4, 1);
+			else if constexpr (sizeof(T) == 4) rc = B200_LN_ROWS(8, 1);
 #undef B200_LN_ROWS
 			partials = rp.grid;
 		}
