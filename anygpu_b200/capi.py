@@ -112,6 +112,7 @@ SIGNATURES = {
     "b200_layer_norm": (_int, [_int, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _f32, _vp]),
     "b200_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "b200_layer_norm_backward": (_int, [_int, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "b200_debug_layer_norm_backward_starved": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_uint32, _vp]),
     "b200_mamba2_decoder_prefill_workspace_bytes": (_sz, [ctypes.POINTER(Mamba2Config), _int, _i64, _i64]),
     "b200_mamba2_decoder_prefill": (_int, [_int, ctypes.POINTER(Mamba2Config), ctypes.POINTER(Mamba2Weights), _vp, _f32, _vp, _vp,
                                            _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),

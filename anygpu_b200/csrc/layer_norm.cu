@@ -307,9 +307,11 @@ __global__ void __launch_bounds__(TPR * ROWS) layer_norm_backward_kernel(const T
 // What bounds the call is how many bytes are on their way per SM; registers that also hold the sums of dw and db have no room for them.
 // A ring of whole rows in shared memory, filled by bulk copies (one instruction per row, completion counted on an mbarrier), has.
 
-__device__ __forceinline__ void row_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err_word)
+__device__ __forceinline__ bool row_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err_word, uint32_t limit)
 {
-	if (!tc::mbar_wait(bar, parity, abort_flag)) tc::report_timeout(err_word, tc::kErrRowWait);
+	const bool filled = tc::mbar_wait(bar, parity, abort_flag, limit);
+	if (!filled) tc::report_timeout(err_word, tc::kErrRowWait);
+	return filled;
 }
 
 // Gradient: a CTA of 256 threads walks groups of R rows; a thread owns NV 16-byte vectors of columns, so dw and db are sums in its
@@ -319,7 +321,7 @@ constexpr int kRowThreads = 256;
 template <typename T, int NV, int R>
 __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x,
 	int64_t xs, const T* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t dxs,
-	float* __restrict__ part, int64_t rows, int dim, int64_t dimp, int stages, uint32_t* err_word)
+	float* __restrict__ part, int64_t rows, int dim, int64_t dimp, int stages, uint32_t* err_word, uint32_t wait_limit)
 {
 	constexpr int V = 16 / sizeof(T), NW = kRowThreads / 32;
 	extern __shared__ __align__(128) unsigned char smem[];  // [stages][R][x | dy][dim]
@@ -335,6 +337,7 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(c
 	}
 	__syncthreads();
 	const int64_t groups = (rows + R - 1) / R;
+	int64_t requests = wait_limit == tc::kSpinLimit ? groups : groups - 1;  // the self-test: a stage that nothing fills
 	auto request = [&](int64_t g, int st) {
 		const int live = rows - g * R < R ? static_cast<int>(rows - g * R) : R;
 		const uint32_t bar = tc::smem_u32(&full[st]);
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(c
 		}
 	};
 	if (threadIdx.x == 0)
-		for (int i = 0; i < stages && blockIdx.x + static_cast<int64_t>(i) * gridDim.x < groups; ++i) request(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
+		for (int i = 0; i < stages && blockIdx.x + static_cast<int64_t>(i) * gridDim.x < requests; ++i) request(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
 	const float inv = 1.f / static_cast<float>(dim);
 	f2 aw[NV][V / 2], ab[NV][V / 2];
 	Pack<T, V> pw[NV];
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(c
 		}
 		if (g + gridDim.x < groups) statistics(g + gridDim.x);
 		const T* stage = reinterpret_cast<const T*>(smem + static_cast<size_t>(st * R * 2) * bytes);
-		row_wait(tc::smem_u32(&full[st]), parity, &abort_flag, err_word);
+		if (!row_wait(tc::smem_u32(&full[st]), parity, &abort_flag, err_word, wait_limit)) requests = 0;
 #pragma unroll
 		for (int r = 0; r < R; ++r)
 		{
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(c
 		}
 		__syncthreads();
 		const int64_t ahead = g + static_cast<int64_t>(stages - 1) * gridDim.x;  // of the stage that the group before this one has left
-		if (threadIdx.x == 0 && g != blockIdx.x && ahead < groups) request(ahead, st == 0 ? stages - 1 : st - 1);
+		if (threadIdx.x == 0 && g != blockIdx.x && ahead < requests) request(ahead, st == 0 ? stages - 1 : st - 1);
 		if (dx)
 #pragma unroll
 			for (int r = 0; r < R; ++r)
@@ -485,6 +488,11 @@ __global__ void __launch_bounds__(kRowThreads) layer_norm_backward_rows_kernel(c
 			st = 0;
 			parity ^= 1;
 		}
+	}
+	if (*reinterpret_cast<volatile int*>(&abort_flag))
+	{
+		// a wait was given up: nothing more was requested, and copies already in flight get time to land before shared memory is released
+		for (int i = 0; i < 2000; ++i) __nanosleep(1000);
 	}
 	if (!part) return;
 	float* pr = part + static_cast<int64_t>(blockIdx.x) * 2 * dimp;
@@ -680,6 +688,9 @@ static int layer_norm_backward_v(const LnPlan& p, const T* dy, int64_t dys, cons
 	});
 }
 
+// The poll limit of the ring's waits; another one (b200_debug_layer_norm_backward_starved) also leaves out the last group's copies.
+static thread_local uint32_t g_row_wait_limit = tc::kSpinLimit;
+
 template <typename T, int NV, int R>
 static int launch_ln_rows_backward(const LnRowsPlan& p, const T* dy, int64_t dys, const T* x, int64_t xs, const T* w, const float* mean,
 	const float* rstd, T* dx, int64_t dxs, float* part, int64_t rows, int dim, int64_t dimp, cudaStream_t st)
@@ -688,7 +699,7 @@ static int launch_ln_rows_backward(const LnRowsPlan& p, const T* dy, int64_t dys
 	B200_CUDA_TRY(allow_dynamic_smem(layer_norm_backward_rows_kernel<T, NV, R>, kRingMax, done));
 	const size_t bytes = static_cast<size_t>(p.ring.stages) * 2 * R * dim * sizeof(T);
 	layer_norm_backward_rows_kernel<T, NV, R><<<p.grid, kRowThreads, bytes, st>>>(dy, dys, x, xs, w, mean, rstd, dx, dxs, part, rows, dim, dimp,
-		p.ring.stages, device_error_word());
+		p.ring.stages, device_error_word(), g_row_wait_limit);
 	B200_LAUNCH_CHECK();
 	return B200_OK;
 }
@@ -799,4 +810,17 @@ extern "C" int b200_layer_norm_backward(int dtype, const void* dy, int64_t dy_st
 	if (dtype == B200_F16)
 		return layer_norm_backward<__half>(dy, dy_stride, x, x_stride, w, mean, rstd, dx, dx_stride, dw, db, rows, dim, part, st);
 	return layer_norm_backward<float>(dy, dy_stride, x, x_stride, w, mean, rstd, dx, dx_stride, dw, db, rows, dim, part, st);
+}
+
+extern "C" int b200_debug_layer_norm_backward_starved(const void* dy, const void* x, const float* mean, const float* rstd, void* dx, int64_t rows,
+	int64_t dim, uint32_t spin_limit, void* stream)
+{
+	if (!dy || !x || !mean || !rstd || !dx) return B200_ERR_NULL;
+	if (rows <= 0 || dim < 1024 || dim > 8192 || dim % 8 != 0 || spin_limit == 0 || spin_limit >= tc::kSpinLimit) return B200_ERR_BAD_SHAPE;
+	if (!aligned16(dy) || !aligned16(x) || !aligned16(dx)) return B200_ERR_MISALIGNED;
+	g_row_wait_limit = spin_limit;
+	const int rc = layer_norm_backward<__half>(dy, dim, x, dim, nullptr, mean, rstd, dx, dim, nullptr, nullptr, rows, dim, nullptr,
+		static_cast<cudaStream_t>(stream));
+	g_row_wait_limit = tc::kSpinLimit;
+	return rc;
 }

@@ -155,6 +155,12 @@ size_t b200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
 int b200_layer_norm_backward(int dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
 	const float* mean, const float* rstd, void* dx, int64_t dx_stride, float* dw, float* db, int64_t rows, int64_t dim,
 	void* workspace, size_t workspace_bytes, void* stream);
+/* Self-test of the give-up path of the gradient's bounded waits, as b200_debug_linear_starved_producer: f16, dense rows, dx only, dim a
+ * multiple of 8 from 1024 to 8192 (the form that streams rows through shared memory). The last rows are never requested and the waits' poll
+ * limit is lowered to `spin_limit`: the kernel records the site in the device error word, lets its copies land and returns. dx holds no
+ * meaningful result. */
+int b200_debug_layer_norm_backward_starved(const void* dy, const void* x, const float* mean, const float* rstd, void* dx, int64_t rows,
+	int64_t dim, uint32_t spin_limit, void* stream);
 
 /* ---- SSD chunked selective scan (prefill) -------------------------------------------------------------------
  * CUDA counterpart of mamba_chunk_scan_combined_ref (scripts/zamba2/mamba_chunk_scan_comb.py:167-215), which anyGPU
