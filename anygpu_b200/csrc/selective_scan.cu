@@ -5,7 +5,7 @@
 //
 // LPC lanes share a channel and own 4 states each, in registers as two packed pairs. A CTA walks its channels in tiles of TT tokens with
 // two kinds of warps, because the two kinds of work wait for different things and hide each other's latency when they run side by
-// side (8192 x 4096 x 16: 267 us with the same warps doing both in turn, 228 us so):
+// side (8192 x 4096 x 16: 267 us with the same warps doing both in turn, 228 us so; 230 with step sizes to two half steps):
 //   * loading warps bring the activations (neighbouring threads, neighbouring channels of a token: a warp that loaded the 16 bytes of its
 //     own channels token by token touched 32 cache lines per access, and the memory pipe was half busy with that), and leave
 //     (delta, delta x) per (channel, token) and the rows of B and C in shared memory, one tile ahead; one tile behind they apply skip

@@ -97,10 +97,11 @@ __device__ __forceinline__ f2 exp_2(f2 v)
 	f = fma2(c, both(kLog2eLow), f);
 	return pow2_split(t, f);
 }
-// The decays of one token. The exponential unit's 2^-22 adds up over a long memory: with it everywhere dA is off by 1.9e-6 and
-// final_state by 4.8e-7 (8192 x 4096 x 16, f16 activations), with the polynomial everywhere by 3.4e-7 and 1.4e-7, at 396 instead of 228 us
-// forward. So fp32 calls, whose results show it, take the polynomial everywhere; f16 calls take it in the adjoint recurrence (dA
-// 9.5e-7; the training step 1250 instead of 1080 us), between segments and for single tokens (64 x 5120 x 16: 15.6 us instead of 14.2).
+// The decays of one token. The exponential unit's 2^-22 adds up over a long memory: with it everywhere dA is off by 1.8e-6 and
+// final_state by 4.7e-7 (8192 x 4096 x 16, f16 activations), with the polynomial everywhere by 3.4e-7 and 1.2e-7, at 406 instead of 230 us
+// forward and 1644 instead of 1275 per training step. So fp32 calls, whose results show it, take the polynomial everywhere; f16 calls take it
+// in the adjoint recurrence (dA 9.5e-7; the training step 1275 instead of 1116 us), between segments and for single tokens (64 x 5120 x 16:
+// 15.7 us instead of 14.4).
 template <bool EXACT>
 __device__ __forceinline__ f2 decay_2(f2 x)
 {

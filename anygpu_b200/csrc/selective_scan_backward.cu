@@ -7,9 +7,9 @@
 // Threads load, lanes own states and warps own channels as in the forward kernel. A CTA walks its tokens backwards in tiles of 16: from the
 // state the forward pass saved before the tile a warp runs the 16 tokens forward once, keeping every state in registers (16 x 4 per lane),
 // then backwards for the adjoint; the decays are computed again on the way back, which costs less than the registers to keep them.
-// 8192 x 4096 x 16 in f16: 1.02 ms. The 128 registers of a thread leave 14 - 16 warps per SM, which is what bounds it: 54% of the issue slots
-// and 58% of the shared-memory pipe are used, a warp waits for fixed latencies 22%, at the two barriers of a tile 14% and for shared
-// memory 11% of its time; HBM stands at 8%.
+// 8192 x 4096 x 16 in f16: 1.04 ms. The 128 registers of a thread leave 14 - 16 warps per SM, which is what bounds it: 55% of the issue slots
+// and 57% of the shared-memory pipe are used, a warp waits for fixed latencies 24%, at the two barriers of a tile 13%, for the multiply-add
+// pipe 11% and for shared memory 10% of its time; HBM stands at 8%.
 // dB and dC need a sum over channels: the lanes of a warp by exchanges, the warps of a CTA through shared memory, the CTAs as partial
 // rows that a second kernel adds; dA, dD and dbias are summed over the tokens where they arise and leave one partial row per (batch
 // entry, segment). No atomics anywhere.

@@ -33,7 +33,8 @@ inline Tensor<dtype, CUDA> tensor_causal_conv1d_update(const Tensor<dtype, CUDA>
 	return y_t;
 }
 
-// Token-major form: xt (batch, seq_len, dims), possibly a last-axis slice view of a wider tensor; zero left padding.
+// Token-major form: xt (batch, seq_len, dims), possibly a last-axis slice view of a wider tensor; zero left padding (states come and go
+// through b200_causal_conv1d_tokens).
 template <typename dtype>
 inline Tensor<dtype, CUDA> tensor_causal_conv1d_tokens(const Tensor<dtype, CUDA>& xt, const Tensor<dtype, CUDA>& wt, const Tensor<dtype, CUDA>& bt)
 {

@@ -218,7 +218,8 @@ int b200_selective_state_update(int dtype, float* ssm_state, const void* x, int6
  * x, dt, z [batch, seqlen, dim] and B, C [batch, seqlen, ngroups, d_state] in dtype, each with its own row (token) stride and a batch
  * stride of seqlen rows; a group serves dim / ngroups consecutive channels. A [dim, d_state] (A_log when a_is_log != 0:
  * A = -exp(A_log)), D [dim] or null, dt_bias [dim] or null, initial_state [batch, dim, d_state] or null (zeros): fp32, contiguous.
- * z null: no gate. d_state <= 128. The state is fp32 throughout. No counterpart in anyGPU. */
+ * z null: no gate. d_state <= 128. The state is fp32 throughout. States, their gradients, checkpoints and the workspace start on 16-byte
+ * boundaries, parameters and activations on any element. No counterpart in anyGPU. */
 typedef struct b200_selective_scan_inputs
 {
 	const void *x, *dt, *B, *C, *z;
