@@ -1,7 +1,8 @@
 // Selective scan with a decay per channel and state (the form of state-space layers before the per-head scan of mamba_chunk_scan.hpp):
-// x, dt, z (b,l,dim), A (dim,n), B/C (b,l,g,n), D and dt_bias (dim), initial_states (b,dim,n); A is A itself and softplus of the step sizes is on (b200_selective_scan has the other forms). A, D,
-// dt_bias and all states are float32. Activations may be last-axis slice views of wider tensors (evenly spaced rows); of B and C that
-// holds for whole rows of g * n elements, not for some of the states of every group. No counterpart in anyGPU.
+// x, dt, z (b,l,dim), A (dim,n), B/C (b,l,g,n), D and dt_bias (dim), initial_states (b,dim,n); A is A itself and softplus of the step sizes
+// is on (b200_selective_scan has the other forms). A, D, dt_bias and all states are float32. Activations may be last-axis slice views of
+// wider tensors (evenly spaced rows); of B and C that holds for whole rows of g * n elements, not for some of the states of every group.
+// No counterpart in anyGPU.
 #pragma once
 
 #include "../b200_call.hpp"
