@@ -48,3 +48,28 @@ def test_checkpoints_are_the_states(ops, n):
         part = {name: v.contiguous() for name, v in part.items()}
         _, want = ref.scan(**reference_args(part))
         ref.assert_within(ck[:, k], want, ref.scan_bounds(**reference_args(part))[1], f"checkpoint {k}")
+
+
+@pytest.mark.parametrize("shape", [(2, 33, 6, 6, 16), (1, 40, 8, 8, 4), (1, 700, 3, 3, 16), (2, 20, 4, 4, 100), (1, 35, 66, 33, 16)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_groups_of_one_and_two_channels(ops, shape, dtype):
+    b, l, d, g, n = shape
+    p, gen = inputs(l + n, b, l, d, g, n, dtype)
+    dy, dfin = rn(gen, b, l, d, dtype=dtype), rn(gen, b, d, n)
+    y, fin, ck = ops.tensor_selective_scan(**p, want_checkpoints=True)
+    grads = ops.tensor_selective_scan_backward(dy, checkpoints=ck, dfinal_states=dfin, **p)
+    leaves = {k: v.requires_grad_() for k, v in reference_args(p).items()}
+    wy, wfin = ref.scan(**leaves)
+    ((wy * dy.double()).sum() + (wfin * dfin.double()).sum()).backward()
+    bounds = ref.scan_bounds(**reference_args(p), dy=dy.double(), dfin=dfin.double())
+    ref.assert_within(y, wy.detach(), bounds[0], "y")
+    ref.assert_within(fin, wfin.detach(), bounds[1], "final_states")
+    for i, (name, leaf) in enumerate(GRADS):
+        ref.assert_within(getattr(grads, name), leaves[leaf].grad, bounds[2 + i], name)
+    state = p["initial_states"].clone()
+    one = {k: (v[:, 0] if k in ("x", "dt", "B", "C", "z") else v) for k, v in p.items() if k != "initial_states"}
+    first = {k: (v[:, :1].contiguous() if k in ("x", "dt", "B", "C", "z") else v) for k, v in p.items()}
+    wy, wfin = ref.scan(**reference_args(first))
+    bounds = ref.scan_bounds(**reference_args(first))
+    ref.assert_within(ops.tensor_selective_scan_update(state, **one), wy[:, 0], bounds[0][:, 0], "single token")
+    ref.assert_within(state, wfin, bounds[1], "state")
